@@ -187,14 +187,16 @@ __global__ void __launch_bounds__(128) short_convolution_kernel(const __grid_con
     constexpr int KEPT = TAPS - 1;
     __shared__ ConvWeights<V, TAPS> weights;
     // The request and tile behind this block's number: request i's tiles begin at cu_q[i] / tile_len + i, which leaves each of them a tile
-    // or more.  Every warp looks at 32 places at a time: 1,024 requests take two loads (a walk over all lengths before a block's request
-    // took 2,000 requests of two tokens x 1,024 channels from 31 to 93 us, 256 x 4,096 from 17 to 21).
+    // or more.  Blocks below the first one's (cu_q[0] rows belong to no request) have nothing to do: they end, since a tile must be one
+    // block's alone.  Every warp looks at 32 places at a time: 1,024 requests take two loads (a walk over all lengths before a block's
+    // request took 2,000 requests of two tokens x 1,024 channels from 31 to 93 us, 256 x 4,096 from 17 to 21).
     int seq = 0, tile = blockIdx.x;
     for (int n = p.n_seqs; n > 1;) {
         const int step = (n + 31) / 32, i = seq + (int)(threadIdx.x & 31) * step;
         const bool there = (int)(threadIdx.x & 31) * step < n;
         const int begin = there ? max(0, min(p.cu_q[i], p.n_tokens)) / tile_len + i : 0;
-        const int k = max(__popc(__ballot_sync(0xffffffffu, there && begin <= (int)blockIdx.x)) - 1, 0);
+        const int k = __popc(__ballot_sync(0xffffffffu, there && begin <= (int)blockIdx.x)) - 1;
+        if (k < 0) return;                      // (the whole block: every warp has looked at the same places)
         tile = max((int)blockIdx.x - __shfl_sync(0xffffffffu, begin, k), 0);
         seq += k * step;
         n = min(step, n - k * step);

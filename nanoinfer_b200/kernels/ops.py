@@ -1005,7 +1005,8 @@ def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torc
 
     x, out [T, D] of one dtype (columns of a wider matrix will do; out apart from x); weight float32 [D, taps] (1 to
     SHORT_CONVOLUTION_MAX_TAPS), the last one the token's own; bias float32 [D] or None.  Request i has rows
-    cu_q[i] .. cu_q[i + 1] (int32 [n_seqs + 1]; none is allowed; rows behind the last request stay as they are), at most
+    cu_q[i] .. cu_q[i + 1] (int32 [n_seqs + 1]; none is allowed; rows before the first request, with cu_q[0] above zero, and
+    behind the last one stay as they are), at most
     ``max_q_len`` of them (None: T; a host's number, so it is taken as given: with too small a one, results are not defined).  What came before them stands in row slots[i] (int32) of ``state``, float32 [slots, *], from column
     ``state_col`` on as [taps - 1, D], oldest first; the last taps - 1 inputs go to row to_slots[i] (default: the same row).
     A slot outside of the state belongs to no request: zeros come from it, nothing is left there.  A row that one request
