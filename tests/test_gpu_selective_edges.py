@@ -69,3 +69,48 @@ def test_the_later_requests_of_a_step():
         ops.short_convolution(x, w, None, state, cu[at:], slots[at:], len(lens) - at, out)
         ops.short_convolution(x, w, None, state, cu, slots, at, out)
         assert torch.equal(out, want) and torch.equal(state, kept), at
+
+
+@pytest.mark.parametrize("n, d", [(1, 40), (5, 33), (16, 40), (16, 33), (8, 64), (64, 16), (128, 24)])
+@pytest.mark.parametrize("form", ["portion", "stepwise", "tokens", "parts"])
+def test_steps_are_as_exact_far_below_zero(form, n, d):
+    """delta alone, all over softplus' range: every other factor is one, nothing is left of the state before and one state is read.
+    In half steps: 2^x is off by 4 (two units in the last place, its documented bound), what the argument's rounding is worth is
+    multiplied in (1), with ln 2 rounded to 1.905e-9 (|v| log2(e) of that, 0.0461 |v|), the polynomial's ten steps leave 2.1 (each
+    rounded at its size, times the powers of e <= 1 behind it, over the smallest value ln 2) and the last sum 1: 8.1 + 0.0461 |v|."""
+    from nanoinfer_b200.kernels import ops
+    g = torch.Generator().manual_seed(n + d)
+    t = {"tokens": 90, "parts": 500}.get(form, 300)
+    low = torch.tensor([-86.0, -20.0, -8.0, -1.0, -0.01, 1.0])
+    high = torch.tensor([-20.0, -8.0, -1.0, 1.0, 0.01, 30.0])
+    which = torch.randint(0, 6, (t, d), generator=g)
+    v = low[which] + (high - low)[which] * torch.rand(t, d, generator=g)
+    v[0, :3] = torch.tensor([0.0, -0.0, -86.0])
+    want = torch.logaddexp(v.double(), torch.zeros((), dtype=torch.float64))
+    one = torch.zeros(t, n)
+    one[:, n // 2] = 1
+    lens = [1] * t if form == "tokens" else [t]
+    out, state = torch.empty(t, d, device=DEV), torch.zeros(t, d * n, device=DEV)
+    ops.selective_scan(torch.ones(t, d, device=DEV), v.to(DEV), torch.full((d, n), -1e38, device=DEV), torch.ones(t, n, device=DEV), one.to(DEV),
+                       state, _cu(lens), _i32(list(range(len(lens)))), len(lens), out, max_q_len=max(lens), stepwise=form == "stepwise")
+    gone = want * 1e38 > 200           # (a decay below e^-200; the smallest steps keep some of the state before)
+    worst = ((out.double().cpu() - want).abs() / (want * (8.1 + 0.0461 * v.double().abs()) * plain.U))[gone].max().item()
+    assert gone.float().mean() > 0.9 and worst <= 1.0, f"{worst:.2f} times the bound"
+
+
+@pytest.mark.parametrize("lens", [[3], [1, 1, 1], [70]])
+def test_steps_that_are_not_finite(lens):
+    """An infinite step where softplus' argument is one, none where it is minus infinity (the state before stays: 4 half steps of 2^x),
+    NaN where it is NaN."""
+    from nanoinfer_b200.kernels import ops
+    t, d = sum(lens), 24
+    v = torch.zeros(t, d)
+    v[1, 4], v[1, 9], v[1, 14] = float("inf"), float("-inf"), float("nan")
+    ones = torch.ones(t, 1, device=DEV)
+    out, state = torch.empty(t, d, device=DEV), torch.zeros(t, d, device=DEV)
+    ops.selective_scan(torch.ones(t, d, device=DEV), v.to(DEV), torch.full((d, 1), -1e38, device=DEV), ones, ones, state, _cu(lens),
+                       _i32(list(range(len(lens)))), len(lens), out, max_q_len=max(lens))
+    row = out[1].cpu()
+    before = out[0, 9].item() if lens[0] > 1 else 0.0
+    assert abs(row[9] - before) <= 4 * plain.U * before
+    assert row[4] == float("inf") and row[14].isnan() and row[[0, 3, 5, 8, 10, 13, 15, 23]].isfinite().all()
