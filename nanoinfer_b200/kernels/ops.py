@@ -897,7 +897,7 @@ _GATE_ACTS = {"none": 0, "identity": 1, "sigmoid": 2, "silu": 3}
 
 _CONV_ARGS = struct.Struct("=8Q3q8i")
 _SCAN_ARGS = struct.Struct("=13Q7q12i")
-_NORMS_ARGS = struct.Struct("=7Q3q5i3f")
+_NORMS_ARGS = struct.Struct("=7Q3q5i4f")
 
 
 def _matrix(t: torch.Tensor, name: str, shape: tuple, device: int, what: str) -> Tuple[int, int, int]:
@@ -1133,7 +1133,7 @@ def add_normed_rmsnorm(h: torch.Tensor, y: torch.Tensor, weight: torch.Tensor, e
         _written_apart(what, n, d, op, o_ld, o_code, read + ((hp, d, F32, d), (to, d, F32, d)))
     _written_apart(what, n, d, to, d, F32, read if to == hp else read + ((hp, d, F32, d),))
     _check(load("block_norms").ni_block_norms(
-        _NORMS_ARGS.pack(hp, to, yp, gp, op, w, g, y_ld, g_ld, o_ld, n, d, code, o_code, act, eps, next_eps, scale),
+        _NORMS_ARGS.pack(hp, to, yp, gp, op, w, g, y_ld, g_ld, o_ld, n, d, code, o_code, act, eps, next_eps, scale, 1.0 / d),
         _stream_of(device, y, what)), what)
 
 
