@@ -529,7 +529,7 @@ class SelectiveStateSpace(Part):
     width, ``state_size`` 16, ``conv_taps`` 4, ``groups`` 1 unless given).
 
     Two launches beside the four products and a copy of dt' (csrc/short_convolution.cu, csrc/selective_scan.cu), for prompt portions
-    and single tokens alike; W_x's and W_dt's results stay FP32 (dt' is rounded for W_dt's product).  A request's state is one FP32 vector: h [channels, state_size], then the last
+    and single tokens alike; W_x's, W_dt's and W_o's results stay FP32 (dt' is rounded for W_dt's product).  A request's state is one FP32 vector: h [channels, state_size], then the last
     conv_taps - 1 inputs of the convolution.  A step's kernels run exactly once, so the state advances by exactly the step's tokens; in
     float32 a token's bits do not depend on how its request is cut into steps."""
 
@@ -599,7 +599,7 @@ class SelectiveStateSpace(Part):
         ops.selective_scan(u, dt, self.a, chosen[:, self.rank:self.rank + gn], chosen[:, self.rank + gn:], cache.state, ctx.cu_q,
                            ctx.slots, ctx.n_seqs, y, skip=self.skip, dt_bias=self.dt_bias, z=proj[:, c:], max_q_len=ctx.max_q_len,
                            stepwise=rt.dtype == f32)
-        return rt.linear(y, self.w_o, residual=residual)
+        return rt.linear(y, self.w_o, out_dtype=f32, residual=residual)
 
 
 register_part("mixer", "matrix_memory", MatrixMemory, replace=True)
