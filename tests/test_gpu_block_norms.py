@@ -62,3 +62,36 @@ def test_rows_beyond_the_numbers():
         h, one = torch.zeros(3, 96, device=DEV), torch.ones(96, device=DEV)
         ops.add_normed_rmsnorm(h, y, one, 0.0, None, 0.0, None)
         assert (h[0] == 0).all() and h[1].isnan().all() and ((h[2] - 1).abs() <= 4 * plain.U).all()
+
+
+# Rows beyond four per SM take eight numbers a thread and share an SM by threes; fewer rows few numbers a thread; widths that no
+# 16-byte piece divides (or columns that begin off one) one number at a time, up to 8,192; wider ones are read twice.
+@pytest.mark.parametrize("act", ["none", "silu", "sigmoid", "identity"])
+@pytest.mark.parametrize("rows, d, left", [(700, 4096, 0), (700, 520, 0), (700, 2044, 0), (1201, 36, 0), (700, 2999, 0), (650, 1024, 1), (3, 6001, 0),
+                                           (601, 8190, 0), (2, 4100, 0), (610, 16380, 0), (593, 5, 0)])
+@pytest.mark.parametrize("y_type, out_type, in_place", [(BF16, BF16, False), (F32, F32, True), (BF16, F32, True)])
+def test_every_form(act, rows, d, left, y_type, out_type, in_place):
+    """Each form of the kernel with a last piece that is not whole, gated and not, against 64 bits; what lies around the columns stays."""
+    from nanoinfer_b200.kernels import ops
+    g = torch.Generator(device=DEV).manual_seed(rows + d)
+
+    def randn(*shape):
+        return torch.randn(*shape, generator=g, device=DEV)
+
+    def columns(t):
+        whole = torch.full((t.shape[0], left + t.shape[1] + left), float("nan"), dtype=t.dtype, device=DEV)
+        whole[:, left:left + t.shape[1]] = t
+        return whole[:, left:left + t.shape[1]]
+
+    h, y, w, gain = randn(rows, d) * 3, columns((randn(rows, d) * 2).to(y_type)), randn(d), randn(d)
+    gate = None if act == "none" else columns(randn(rows, d).to(y_type))
+    want, err, new, new_err = plain.norms(h, y, w, 1e-5, gain, 1e-6, 0.37, gate, act)
+    stream, h_out = h.clone(), torch.full_like(h, 7.0)
+    out = columns(torch.zeros(rows, d, dtype=out_type, device=DEV))
+    ops.add_normed_rmsnorm(stream, y, w, 1e-5, gain, 1e-6, out, scale=0.37, gate=gate, gate_act=act, h_out=None if in_place else h_out)
+    if not in_place:
+        assert torch.equal(stream, h)
+    for got, exact, bound, kind in ((stream if in_place else h_out, new, new_err, F32), (out, want, err, out_type)):
+        worst = ((got.double() - exact).abs() / (bound + plain.half_step(kind) * (exact.abs() + bound) + 1e-37)).max().item()
+        assert worst <= 1.0, f"{worst:.2f} times the bound"
+    assert out._base is None or not left or (out._base[:, :left].isnan().all() and out._base[:, -left:].isnan().all())

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 import plain_selective as plain
-from test_gpu_selective import BF16, DEV, F32, _close, _conv_case, _cu, _i32, _scan_case
+from test_gpu_selective import BF16, DEV, F32, _close, _conv_case, _cu, _i32, _scan, _scan_case
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +114,40 @@ def test_steps_that_are_not_finite(lens):
     before = out[0, 9].item() if lens[0] > 1 else 0.0
     assert abs(row[9] - before) <= 4 * plain.U * before
     assert row[4] == float("inf") and row[14].isnan() and row[[0, 3, 5, 8, 10, 13, 15, 23]].isfinite().all()
+
+
+@pytest.mark.parametrize("count, d, n, groups", [(61, 8192, 16, 1), (50, 8200, 16, 1), (40, 16384, 8, 1), (61, 4096, 32, 2), (61, 2048, 64, 4),
+                                                 (61, 1024, 128, 1), (130, 40, 16, 1)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_single_tokens_in_many_groups(count, d, n, groups, dtype):
+    """So many requests of one token for their channels that a block walks several groups of them, past those whose states are on
+    their way from the start; some have no tokens, some no row to come from or to go to."""
+    from nanoinfer_b200.kernels import ops
+    lens = [1] * count
+    for i in (3, 10, count - 2):
+        lens[i] = 0
+    k = _scan_case(lens, d, n, groups, dtype, d + n)
+    rows = len(k["state"])
+    k["slots"] = [(-1 if i % 11 == 4 else rows + 3 if i % 11 == 9 else v) for i, v in enumerate(k["slots"])]
+    k["to"] = [(-2 if i % 13 == 6 else rows if i % 13 == 12 else v) for i, v in enumerate(k["to"])]
+    for in_place in (False, True):
+        to = k["slots"] if in_place else k["to"]
+        want, err, new, new_err = plain.scan(k["u"], k["dt"], k["a"], k["b"], k["c"], k["state"], lens, k["slots"], to, k["skip"], k["dt_bias"], k["z"])
+        out, state = _scan(ops, k, lens, in_place)
+        _close(out, want, err, dtype, "out")
+        _close(state, new, new_err, F32, "state")
+
+
+@pytest.mark.parametrize("lens", [[173], [40, 0, 205]])
+@pytest.mark.parametrize("d, n", [(8192, 16), (8200, 16), (4096, 16), (1024, 64), (640, 128), (4096, 8), (2048, 32)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_tiles_of_many_channels(lens, d, n, dtype):
+    """Enough tiles that each of a block's two buffers is filled several times, and a last one that is not whole, in blocks of every
+    number of channels and lanes (64 channels of 16 states where there are many)."""
+    from nanoinfer_b200.kernels import ops
+    k = _scan_case(lens, d, n, 1, dtype, d + n)
+    want, err, new, new_err = plain.scan(k["u"], k["dt"], k["a"], k["b"], k["c"], k["state"], lens, k["slots"], k["to"], k["skip"], k["dt_bias"], k["z"])
+    for given in (dict(), dict(stepwise=True)) if dtype == F32 else (dict(),):
+        out, state = _scan(ops, k, lens, **given)
+        _close(out, want, err, dtype, "out")
+        _close(state, new, new_err, F32, "state")
