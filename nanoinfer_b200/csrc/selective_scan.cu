@@ -282,7 +282,7 @@ static bool ss_wide(const void* p, long long ld, int type, int step) {
 // states leave (ScanBuffer) of the one before that.
 //
 // Bound by neither bytes nor 2^x alone (a state's step: one 2^x, four multiply-adds, a fourth of two 16-byte reads of shared memory):
-// 2,048 tokens x 4,096 channels x 16 states in bfloat16 77 us (13 by its bytes, 30 by 2^x), 8,192 x 8,192 513 (103; 239).  One scanning
+// 2,048 tokens x 4,096 channels x 16 states in bfloat16 79 us (13 by its bytes, 30 by 2^x), 8,192 x 8,192 519 (103; 239).  One scanning
 // warp per scheduler waits on the length of its own chain; with two the reads of B and C from shared memory fill that unit to 85 %.
 // Within a tile a decay is one 2^x, off to one side by up to 0.25 x 2^-24 where it is near one; what the tile's first state is
 // worth at its end is put right by the decay over the whole tile, from the sum of its deltas (the product of the tile's decays is
@@ -849,7 +849,8 @@ __global__ void __launch_bounds__(SS_TOKEN_THREADS, 5) selective_tokens_kernel(c
     }
 }
 
-// The same for numbers of states and addresses that 16-byte pieces do not fit.
+// The same for numbers of states and addresses that 16-byte pieces do not fit.  Bound by its loads, number by number: 128 requests x 8,192
+// channels x 5 states 21.7 us (8 by their bytes).
 template <typename TU, int LANES>
 __global__ void __launch_bounds__(256) selective_token_kernel(const __grid_constant__ ScanArgs p) {
     constexpr int NS = 4, GROUP = ScanGroup<LANES>::N;
